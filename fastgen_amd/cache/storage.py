@@ -17,12 +17,25 @@ row is nobody's: stand-in sequences of a captured step use it).
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import Dict, List, Optional, Sequence, Tuple
+from typing import Dict, List, Optional, Sequence, Tuple, Union
 
 import torch
 
 from .layout import E4M3_BLOCK
 from ..parts.base import LayerStore, PagedNeed, StateNeed
+
+
+# what a cache holds, by name: the model's dtype (None), or 8 bits
+KV_DTYPES: Dict[str, Optional[torch.dtype]] = {"model": None, "e4m3": torch.float8_e4m3fn}
+
+
+def kv_dtype_of(what: Union[str, torch.dtype, None]) -> Optional[torch.dtype]:
+    """A cache's dtype from its name in :data:`KV_DTYPES`; a dtype (or None) is itself."""
+    if not isinstance(what, str):
+        return what
+    if what not in KV_DTYPES:
+        raise ValueError(f"a cache of {what!r}: its names are {', '.join(sorted(KV_DTYPES))}")
+    return KV_DTYPES[what]
 
 
 @dataclass(frozen=True)

@@ -12,7 +12,7 @@ import os
 import time
 from dataclasses import dataclass
 from pathlib import Path
-from typing import Any, Dict, Hashable, List, Mapping, Optional, Sequence
+from typing import Any, Dict, Hashable, List, Mapping, Optional, Sequence, Union
 
 import torch
 
@@ -91,7 +91,7 @@ class Engine:
                  max_step_tokens: int = 2048, max_seq: Optional[int] = None, seed: int = 0,
                  sync_freq: int = 10, overlap_steps: Optional[bool] = None,
                  reserve_bytes: Optional[int] = None, admit_reserve: int = 128,
-                 kv_dtype: Optional[torch.dtype] = None) -> None:
+                 kv_dtype: Union[str, torch.dtype, None] = None) -> None:
         """``max_tokens``: the cache's size in tokens; None: whatever memory the device has free
         now, the weights being in place, beside ``reserve_bytes`` (default: an estimate of what a
         step of ``max_step_tokens`` tokens and ``max_batch`` rows of logits take, plus 2 GiB).

@@ -16,13 +16,13 @@ from typing import IO, Optional
 
 import torch
 
+from ..cache.storage import KV_DTYPES
 from ..config import read_config_json
 from .context import StepEntry
 from .model import Model
 from .runner import ModelRunner
 
 DTYPES = {"bfloat16": torch.bfloat16, "float32": torch.float32}
-KV_DTYPES = {"model": None, "e4m3": torch.float8_e4m3fn}
 
 
 def replay(model_dir: str, dtype: str, out_dir: str, max_tokens: int, page_size: int = 64,
@@ -47,7 +47,7 @@ def replay(model_dir: str, dtype: str, out_dir: str, max_tokens: int, page_size:
     # each request's count is rounded up to whole pages of at least 64 tokens
     unit = max(64, page_size)
     pool_tokens = -(-max_tokens // unit) * unit
-    runner = ModelRunner(model, page_size=page_size, max_tokens=pool_tokens, max_requests=max_live, kv_dtype=KV_DTYPES[kv_cache])
+    runner = ModelRunner(model, page_size=page_size, max_tokens=pool_tokens, max_requests=max_live, kv_dtype=kv_cache)
     for line in stdin:
         line = line.strip()
         if not line:

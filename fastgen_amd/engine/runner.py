@@ -12,12 +12,12 @@ from __future__ import annotations
 
 import logging
 import os
-from typing import Dict, Hashable, Optional, Sequence, Tuple
+from typing import Dict, Hashable, Optional, Sequence, Tuple, Union
 
 import torch
 
 from ..cache.manager import CacheManager
-from ..cache.storage import CacheStorage, group_entries, tokens_for_free_memory
+from ..cache.storage import CacheStorage, group_entries, kv_dtype_of, tokens_for_free_memory
 from ..kernels.ops import E4M3_BLOCK, upload
 from .context import StepContext, StepEntry, build_context, context_from_packed, pack_context
 from .model import Model
@@ -123,15 +123,15 @@ class ModelRunner:
     (each live request's length counts rounded up to whole pages); None: as
     many as the device's free memory holds beside ``reserve_bytes``, at most
     ``at_most_tokens``.  ``max_requests`` is the number of state slots.
-    ``kv_dtype``: what the cache holds, the model's dtype (None) or
-    ``torch.float8_e4m3fn``: 8 bits with a scale for 32 tokens of a kv head
+    ``kv_dtype``: what the cache holds, the model's dtype (None or "model") or
+    ``torch.float8_e4m3fn`` ("e4m3"): 8 bits with a scale for 32 tokens of a kv head
     (:mod:`fastgen_amd.kernels.cache_e4m3`), for bfloat16 models whose
     attention layers all run over it and pages of a multiple of 32 tokens.
     """
 
     def __init__(self, model: Model, page_size: int = 64, max_tokens: Optional[int] = 4096, max_requests: int = 64,
                  pages_per_group: Optional[Sequence[int]] = None, reserve_bytes: int = 2 << 30,
-                 at_most_tokens: Optional[int] = None, kv_dtype: Optional[torch.dtype] = None) -> None:
+                 at_most_tokens: Optional[int] = None, kv_dtype: Union[str, torch.dtype, None] = None) -> None:
         self.model = model
         self.page_size = page_size
         self.kv_dtype = self._checked_kv_dtype(kv_dtype)
@@ -165,8 +165,8 @@ class ModelRunner:
                     "recorded as graphs" if self.use_graphs else "run eagerly")
         self.run_ahead = 16  # steps the host may prepare before the device has run them
 
-    def _checked_kv_dtype(self, kv_dtype: Optional[torch.dtype]) -> torch.dtype:
-        model = self.model
+    def _checked_kv_dtype(self, kv_dtype: Union[str, torch.dtype, None]) -> torch.dtype:
+        model, kv_dtype = self.model, kv_dtype_of(kv_dtype)
         if kv_dtype in (None, model.dtype):
             return model.dtype
         if kv_dtype != torch.float8_e4m3fn or model.dtype != torch.bfloat16:

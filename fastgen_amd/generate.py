@@ -17,11 +17,11 @@ import queue
 import weakref
 from dataclasses import dataclass, field
 from pathlib import Path
-from typing import Any, Iterator, List, Optional, Sequence
+from typing import Any, Iterator, List, Optional, Sequence, Union
 
 import torch
 
-from .cache.storage import bytes_per_token, group_entries
+from .cache.storage import bytes_per_token, group_entries, kv_dtype_of
 from .engine import Engine, Model
 from .engine.trace_window import TraceWindow
 from .sampling import SamplingParams
@@ -52,8 +52,8 @@ class GenArgs:
     sync_freq: int = 10  # decode steps between host checks for finished requests (when nobody waits)
     seed: int = 777  # the reference's tools seed the global generator with 777 (tools/chat.py:47)
     dtype: torch.dtype = torch.bfloat16
-    # beyond the reference: the cache in 8 bits (torch.float8_e4m3fn; None: in `dtype`), weights in 4 bits (the k of a group; 0: in `dtype`)
-    kv_dtype: Optional[torch.dtype] = None
+    # beyond the reference: the cache in 8 bits ("e4m3" or torch.float8_e4m3fn; None or "model": in `dtype`), weights in 4 bits (the k of a group; 0: in `dtype`)
+    kv_dtype: Union[str, torch.dtype, None] = None
     w4_group: int = 0
 
 
@@ -185,6 +185,7 @@ class Fastgen:
         if stop_tokens is None:
             eos = getattr(model.args, "extra", {}).get("eos_token_id", [])
             stop_tokens = eos if isinstance(eos, (list, tuple)) else [eos]
+        kv_dtype = kv_dtype_of(gen_args.kv_dtype)
         max_tokens: Optional[int] = gen_args.max_seq
         if num_pages is not None:
             if num_pages < 1:
@@ -192,7 +193,7 @@ class Fastgen:
             max_tokens = num_pages * gen_args.cache_block
         elif gen_args.max_seq < 0:
             if gen_args.gpu_gb > 0:
-                per_token = bytes_per_token(group_entries(model.paged_needs()), gen_args.kv_dtype or gen_args.dtype)
+                per_token = bytes_per_token(group_entries(model.paged_needs()), kv_dtype or gen_args.dtype)
                 max_tokens = cache_tokens_for_budget(model, gen_args, per_token)
             else:
                 max_tokens = None  # the engine takes what is free
@@ -202,7 +203,7 @@ class Fastgen:
         engine = Engine(model, page_size=gen_args.cache_block, max_tokens=max_tokens, max_batch=max_batch,
                         max_step_tokens=gen_args.max_prefill, max_seq=max_tokens, seed=gen_args.seed,
                         sync_freq=gen_args.sync_freq, reserve_bytes=int(gen_args.prefill_gb * 1e9) + (2 << 30)
-                        if max_tokens is None else None, kv_dtype=gen_args.kv_dtype)
+                        if max_tokens is None else None, kv_dtype=kv_dtype)
         logger.info("cache of %d tokens in pages of %d, at most %d requests",
                     engine.scheduler.pool_tokens, gen_args.cache_block, engine.scheduler.max_batch)
         engine.runner.max_graphs = max(0, gen_args.num_cuda_graphs)

@@ -78,7 +78,7 @@ def main(argv: Optional[List[str]] = None) -> int:
         use_sampling=bool(a.temperature), temperature=a.temperature, top_p=a.top_p, max_batch=1,
         max_gen=a.max_tokens, gpu_gb=a.gpu_gb, cache_block=a.page_size, max_seq=a.max_seq,
         max_prefill=a.max_step_tokens, seed=a.seed, dtype=getattr(torch, a.dtype),
-        kv_dtype=torch.float8_e4m3fn if a.kv_cache == "e4m3" else None, w4_group=a.weights_4_bit,
+        kv_dtype=a.kv_cache, w4_group=a.weights_4_bit,
     )
     stop_tokens = tokenizer.stop_tokens if tokenizer else None
     if a.random_weights is not None:
