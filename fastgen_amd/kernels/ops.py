@@ -656,10 +656,9 @@ def _split_target_blocks() -> int:
     to eight times as many tried at batch 1, 8 and 64).  The splits' partial results are merged by a second
     kernel: merging them in the split that finishes last needs device-scope fences, which on a GPU of
     several dies cost more than the launch they save (measured)."""
-    return _SPLIT_TARGET or compute_units()
+    env = os.environ.get("FG_SPLIT_TARGET")
+    return int(env) if env else compute_units()
 
-
-_SPLIT_TARGET = int(os.environ.get("FG_SPLIT_TARGET") or 0)
 
 # a chunk of the decode attention's key ranges is a multiple of this many 64-key tiles (one a wave)
 _SPLIT_MIN_TILES = int(os.environ.get("FG_SPLIT_MIN_TILES", 4))
