@@ -184,8 +184,9 @@ def _goes_large(M: int, N: int, K: int, ldx: int) -> bool:
 
 
 def w4_scratch(M: int, N: int) -> int:
-    """Bytes that the sums of cuts of K take at most for up to ``M`` rows: 16 cuts, a workgroup of 128 columns x 64 rows a compute unit, or those of the large tiles."""
-    return max(min(_MAX_SPLITS * M * N, 128 * 64 * ops.compute_units()) * 4, ops.gemm_large_scratch(M, N) if M > DIRECT_ROWS else 0)
+    """Bytes that the sums of cuts of K take at most for up to ``M`` rows: 16 cuts, a workgroup (up to 256 columns x 64 rows, :func:`w4_plan`) a compute unit, or
+    those of the large tiles."""
+    return max(min(_MAX_SPLITS * M * N, 256 * 64 * ops.compute_units()) * 4, ops.gemm_large_scratch(M, N) if M > DIRECT_ROWS else 0)
 
 
 def gemm_w4(x, w: Weight4, out_dtype: Optional[torch.dtype] = None, silu_mul_epilogue: bool = False, leave_sums: bool = False) -> torch.Tensor:
