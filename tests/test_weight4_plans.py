@@ -1,8 +1,12 @@
 """How the products with weights in 4 bits are cut (CPU), and every form of the kernel for 17 and more rows (GPU)."""
 
 import pytest
+import torch
+
+from test_weight4 import DEV, _in_64, _matrix, _to, _x, gpu
 
 from fastgen_amd.kernels import ops, weight4
+from fastgen_amd.kernels.weight4 import gemm_w4, pack_w4
 
 ROWS = (*range(17, 97), 100, 127, 128, 129, 192, 257, 700, 2048, 8192)
 COLUMNS = (16, 48, 1000, 1024, 4096, 6144, 11264, 14336, 25600, 28672, 29536, 57344, 128000)
@@ -49,3 +53,62 @@ def test_sums_of_two_blocks_a_wave(units):
     """Two cuts of 64 rows of 28,672 columns: workgroups of 256 columns."""
     assert weight4.w4_plan(64, 28672, 4096, 128) == (4, 2, 2)
     assert weight4.w4_scratch(64, 28672) >= 2 * 64 * 28672 * 4
+
+
+# ------------------------------------------------------------------------------- GPU
+# columns: a wave's second block partly or wholly behind the end, a last block of 8 rows; k of whole and of cut blocks of 128
+SHAPES = {32: [(1000, 1184), (48, 800)], 64: [(1000, 1088), (272, 1024)], 128: [(1000, 1280), (272, 1152), (48, 1024)]}
+
+
+@gpu
+@pytest.mark.parametrize("group,mb,nt", [(g, mb, nt) for g in weight4.GROUPS for mb, nt in sorted(_forms(g))])
+def test_every_form(monkeypatch, group, mb, nt):
+    """Rows of one workgroup and of several, the last of them full, of one row and of all but one; K whole and cut; every kind of result."""
+    for n, k in SHAPES[group]:
+        w = pack_w4(*_matrix(n + k + group, n, k, group))
+        blocks = -(-k // 128)
+        for m in (17, 16 * mb - 1, 16 * mb, 16 * mb + 1, 96):
+            x = _x(m, m, k, 8)[:, :k]
+            want, tol = _in_64(x, w, out_half=0.0)
+            gated, gated_tol = _in_64(x, w, gated=True) if n % 16 == 0 else (None, None)
+            x = x.to(DEV)
+            for splits in (1, 2, 3, blocks):
+                if -(-blocks // splits) * (splits - 1) >= blocks:
+                    continue
+                monkeypatch.setattr(weight4, "w4_plan", lambda *a: (mb, nt, splits))
+                where = f"[{m}, {k}] x [{n}, {k}] in {splits} cuts"
+                for out, half in ((torch.bfloat16, 2.0**-8), (torch.float32, 2.0**-24)):
+                    got = gemm_w4(x, _to(w, DEV), out)
+                    assert got.dtype == out and got.shape == (m, n)
+                    assert ((got.cpu().double() - want).abs() <= tol + half * (want.abs() + tol)).all(), f"{where}: {out}"
+                if n % 16:
+                    continue
+                sums = gemm_w4(x, _to(w, DEV), leave_sums=True)
+                assert sums.shape == ((splits, m, n) if splits > 1 else (m, n))
+                if splits > 1:
+                    assert ((sums.cpu().double().sum(0) - want).abs() <= tol).all(), f"{where}: sums"
+                got = gemm_w4(x, _to(w, DEV), silu_mul_epilogue=True)
+                assert got.shape == (m, n // 2) and ((got.cpu().double() - gated).abs() <= gated_tol).all(), f"{where}: gated"
+
+
+@gpu
+@pytest.mark.parametrize("group", [64, 128])
+def test_two_blocks_a_wave_have_the_bits_of_one(monkeypatch, group):
+    n, k = 1008, 1280
+    w, x = _to(pack_w4(*_matrix(group, n, k, group)), DEV), _x(5, 48, k).to(DEV)
+    found = []
+    for nt in (1, 2):
+        monkeypatch.setattr(weight4, "w4_plan", lambda *a: (3, nt, 2))
+        found.append([gemm_w4(x, w, torch.float32), gemm_w4(x, w, silu_mul_epilogue=True), gemm_w4(x, w, leave_sums=True)])
+    assert all(torch.equal(a, b) for a, b in zip(*found))
+
+
+@gpu
+@pytest.mark.parametrize("n,k,group,m", [(28672, 256, 128, 60), (28672, 256, 64, 33), (28672, 256, 32, 64), (28672, 2176, 128, 64)])
+def test_wide_matrices_as_they_are_planned(n, k, group, m):
+    """Of so many columns a wave takes two blocks, with groups of 32 one."""
+    w = pack_w4(*_matrix(n, n, k, group))
+    assert weight4.w4_plan(m, n, k, group)[1] == (1 if group == 32 else 2)
+    x = _x(m, m, k)
+    want, tol = _in_64(x, w, gated=True)
+    assert ((gemm_w4(x.to(DEV), _to(w, DEV), silu_mul_epilogue=True).cpu().double() - want).abs() <= tol).all()
