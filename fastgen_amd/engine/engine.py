@@ -17,7 +17,6 @@ from typing import Any, Dict, Hashable, List, Mapping, Optional, Sequence, Union
 import torch
 
 from ..kernels.ops import gemm_f32_scratch, gemm_large_scratch, key_parts_scratch
-from ..kernels.linear import Matrix4
 from ..sampling import Sampler, SamplingParams
 from .context import StepEntry
 from .model import Model
@@ -60,10 +59,9 @@ def step_memory_estimate(model: Model, max_step_tokens: int, max_batch: int) -> 
                 if v.dtype == torch.float32:
                     cut = 6 * (-(-max_step_tokens // 16) * 16) * shape[1] if getattr(v, "cut", None) is not None else 0  # x in its parts
                     scratch = max(scratch, gemm_f32_scratch(max_step_tokens, *shape) + cut)
-                elif isinstance(v, Matrix4):
-                    scratch = max(scratch, v.scratch_bytes(max_step_tokens))
                 elif getattr(v, "packed", None) is not None:
                     scratch = max(scratch, gemm_large_scratch(max_step_tokens, shape[0]))
+    scratch = max([scratch] + [m.scratch_bytes(max_step_tokens) for m in model.matrices4()])
     return int(max_step_tokens * 12 * widest + 3 * max_batch * model.vocab_size * 4) + scratch
 
 

@@ -20,7 +20,7 @@ from ..config import ModelLayout, PartSpec, get_architecture, read_config_json
 from ..kernels.linear import Matrix4, StreamedMatrix, four_bits, packing, packing_fits
 from ..kernels.ops import (PackedExperts, PostNormed, ScaledDelta, ScaledRows, StreamTerms, post_add_rmsnorm, stream_add, stream_terms,
                            streams_spread)
-from ..parts import LayerStore, PagedNeed, StateNeed, TensorSpec, build_part
+from ..parts import LayerStore, PagedNeed, Part, StateNeed, TensorSpec, build_part
 from ..parts.base import MATRIX
 from ..weights.source import RandomSource, SafetensorsSource, TensorSource, check_against_specs
 from .context import StepContext
@@ -139,7 +139,7 @@ class Model:
                 part.load(tensors, self.dtype, self.device)
             if getattr(self.parts.head, "tied_to", None):
                 self.parts.head.tie(self.parts.embed.weight)
-        if self.w4_group and not any(isinstance(v, Matrix4) for p in self.parts.all_parts for v in vars(p).values()):
+        if self.w4_group and not self.matrices4():
             raise ValueError(f"no matrix of this model can be in 4 bits in groups of {self.w4_group}: those of plain attention and gated"
                              " feed-forward layers whose width the group divides")
         self.loaded = True
@@ -163,6 +163,12 @@ class Model:
     def capturable(self) -> bool:
         """Whether every part's forward may be recorded into a HIP graph."""
         return all(getattr(p, "capturable", True) for p in self.parts.all_parts)
+
+    def matrices4(self) -> List[Matrix4]:
+        """The matrices in 4 bits, those of a part's own parts (a mixture's shared expert) among them, each once."""
+        inner = [v for p in self.parts.all_parts for v in vars(p).values() if isinstance(v, Part)]
+        found = (v for p in self.parts.all_parts + inner for v in vars(p).values() if isinstance(v, Matrix4))
+        return list({id(v): v for v in found}.values())
 
     def packed(self) -> bool:
         """Whether the matrices have their second copy in the streaming kernels' order."""
