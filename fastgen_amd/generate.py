@@ -52,7 +52,7 @@ class GenArgs:
     sync_freq: int = 10  # decode steps between host checks for finished requests (when nobody waits)
     seed: int = 777  # the reference's tools seed the global generator with 777 (tools/chat.py:47)
     dtype: torch.dtype = torch.bfloat16
-    # beyond the reference: the cache in 8 bits ("e4m3" or torch.float8_e4m3fn; None or "model": in `dtype`), weights in 4 bits (the k of a group; 0: in `dtype`)
+    # beyond the reference: the cache in 8 bits ("e4m3" or torch.float8_e4m3fn; None or "model": in `dtype`), weights in 4 bits (the k of a group; 0: in `dtype`, or as a model that is there already has them)
     kv_dtype: Union[str, torch.dtype, None] = None
     w4_group: int = 0
 
@@ -185,6 +185,10 @@ class Fastgen:
         if stop_tokens is None:
             eos = getattr(model.args, "extra", {}).get("eos_token_id", [])
             stop_tokens = eos if isinstance(eos, (list, tuple)) else [eos]
+        if gen_args.w4_group and gen_args.w4_group != model.w4_group:
+            raise ValueError(f"w4_group={gen_args.w4_group}: the model is there already, with weights "
+                             + (f"in 4 bits in groups of {model.w4_group}" if model.w4_group else f"of {model.dtype}")
+                             + f"; Model.from_folder(..., w4_group={gen_args.w4_group}) makes one in groups of {gen_args.w4_group}")
         kv_dtype = kv_dtype_of(gen_args.kv_dtype)
         max_tokens: Optional[int] = gen_args.max_seq
         if num_pages is not None:

@@ -162,3 +162,19 @@ def test_a_mixture_whose_shared_expert_is_in_4_bits(tmp_path):
     trace = traces.tail(lengths)
     got = run_trace(ModelRunner(model, page_size=16, max_tokens=traces.max_live_tokens(trace, round_to=64), max_requests=4), trace, tokens)
     _close_to_plain(got, want, noise, torch.bfloat16, "shared experts in 4 bits", True)
+
+
+def test_arguments_that_ask_for_other_weights_than_the_model_has(model, monkeypatch):
+    """A model that is there already keeps its weights: arguments that ask for others are refused; those that say nothing take it as it is."""
+    from fastgen_amd.engine import Model
+
+    from fastgen_amd.kernels import ops
+
+    monkeypatch.setattr(ops, "compute_units", lambda: 256)
+    with pytest.raises(ValueError, match="groups of 32"):
+        Fastgen.from_model(model, GenArgs(w4_group=32, max_seq=256), ())
+    small = Model.random(TINY, 1, torch.bfloat16, "cpu", w4_group=32)
+    with pytest.raises(ValueError, match="groups of 64"):
+        Fastgen.from_model(small, GenArgs(w4_group=64, max_seq=256), ())
+    for args in (GenArgs(max_seq=256), GenArgs(w4_group=32, max_seq=256)):
+        assert Fastgen.from_model(small, args, ()).engine.model is small
