@@ -419,12 +419,16 @@ __global__ __launch_bounds__(256) void w4_half_kernel(const bf16_t* __restrict__
   }
 }
 
-// Up to 16 rows.  us by blocks of 16 rows of W, of 4,096 k and more: 256 (4,096 rows) with one, two and four a workgroup 4.5 / 5.6 / 8.3 at one row of x, 384 9.0 / 8.3 / 11
-// at 16 rows, 512 x 28,672 k 36.0 / 34.9 / 39, 1,792 18.4 / 16.9 / 17.3 at 8 rows and - / 21 / 19.1 at 16, whose x the blocks share.  Two blocks a workgroup with
-// 16 waves of one block of k and with 8 of two, 1 / 8 / 16 rows: 384 x 4,096 k 5.8 / 6.3 / 7.6 and 6.0 / 6.3 / 7.5, 704 x 2,048 k 6.9 / 7.7 / 8.9 and 5.5 / 6.2 / 7.4, 1,024 x
-// 2,048 k 7.7 / 8.4 / 9.7 and 6.2 / 6.8 / 8.0.  One block a workgroup with two blocks of k a wave and with one, 1 / 8 / 16 rows: 320 x 5,120 k 9.9 / 11.2 / 14.9 and 8.2 / 9.8 /
-// 13.4 (two workgroups share a unit), 256 x 4,096 k 5.3 / 6.0 / 7.2 and 5.3 / 5.7 / 6.9, x 8,192 k 8.0 / 8.9 / 11.9 and 8.1 / 8.9 / 10.9, x 14,336 k 11.3 / 12.9 / 18.8 and 12.2 / 13.3 /
-// 16.9 (that in groups of 64 13.6 / 15.1 / 19.9 and 12.9 / 13.9 / 19.5).  (The number of rows picks nothing: a row has the same bits whatever is beside it.)
+// Up to 16 rows.  A workgroup has one block of 16 rows of W up to as many workgroups as there are compute units (256), with groups of 32 up to three a unit, two blocks up to
+// 1,024 blocks, then four.  us at 1 / 8 / 16 rows with one block and with two, groups of 128: 256 blocks x 5,120 k 6.2 / 6.8 / 8.3 and 8.2 / 9.0 / 10.2, 288 8.2 / 9.8 / 13.5 and 8.3 / 9.0 /
+// 10.2, 512 8.8 / 10.1 / 13.8 and 8.9 / 9.4 / 10.6; x 2,048 k 256 3.6 / 4.0 / 4.6 and 4.0 / 4.3 / 4.9, 288 4.5 / 5.3 / 6.6 and 4.1 / 4.3 / 4.9; x 8,192 k 256 8.2 / 9.0 / 10.9 and 11.5 / 11.8 / 13.6,
+// 288 12.0 / 14.4 / 19.0 and 11.8 / 11.9 / 13.7.  Groups of 64: 256 x 5,120 k 6.3 / 7.1 / 9.0 and 7.5 / 8.3 / 10.3, 288 10.0 / 11.5 / 15.4 and 7.6 / 8.5 / 10.6.  Groups of 32: 256 x 5,120 k 7.1 / 7.6 / 9.3
+// and 15.4 / 16.4 / 17.6, 768 17.8 / 19.2 / 24.0 and 20.1 / 21.5 / 23.9, 896 21.9 / 23.9 / 30.1 and 20.3 / 21.8 / 24.1 (768 x 2,048 k 9.9 / 10.7 / 12.4 and 9.7 / 10.2 / 11.3).  Two and four blocks: 1,792 x 4,096 k
+// 16.9 and 17.3 at 8 rows, 21 and 19.1 at 16, whose x the blocks share; 512 x 28,672 k 34.9 and 39 at 8.
+// Two blocks a workgroup with 16 waves of one block of k and with 8 of two, 1 / 8 / 16 rows: 384 x 4,096 k 5.8 / 6.3 / 7.6 and 6.0 / 6.3 / 7.5, 704 x 2,048 k 6.9 / 7.7 / 8.9 and 5.5 / 6.2 / 7.4, 1,024 x
+// 2,048 k 7.7 / 8.4 / 9.7 and 6.2 / 6.8 / 8.0.  One block a workgroup with two blocks of k a wave and with one: 256 x 4,096 k 5.3 / 6.0 / 7.2 and 5.3 / 5.7 / 6.9, x 8,192 k 8.0 / 8.9 / 11.9 and
+// 8.1 / 8.9 / 10.9, x 14,336 k 11.3 / 12.9 / 18.8 and 12.2 / 13.3 / 16.9 (that in groups of 64 13.6 / 15.1 / 19.9 and 12.9 / 13.9 / 19.5).  (The number of rows picks nothing: a row has the same bits whatever
+// is beside it.)
 template <int GROUP, int EPI, class OUT>
 static void launch_rows(const W4Args& a, const RowScale& sc, const Residual& rs, hipStream_t stream) {
   const int nb = (a.N + 15) / 16;
@@ -434,7 +438,7 @@ static void launch_rows(const W4Args& a, const RowScale& sc, const Residual& rs,
       w4_rows_kernel<1, 2, 16, false, GROUP, EPI, OUT><<<nb, 1024, 0, stream>>>(a, sc, rs);
       return;
     }
-  if (nb <= 320) w4_rows_kernel<1, 1, 16, false, GROUP, EPI, OUT><<<nb, 1024, 0, stream>>>(a, sc, rs);
+  if (nb <= (GROUP == 32 ? 768 : 256)) w4_rows_kernel<1, 1, 16, false, GROUP, EPI, OUT><<<nb, 1024, 0, stream>>>(a, sc, rs);
   else if (nb <= 1024) w4_rows_kernel<2, GROUP == 128 ? 2 : 1, WAVES, GROUP != 32, GROUP, EPI, OUT><<<(nb + 1) / 2, WAVES * FG_WAVE, 0, stream>>>(a, sc, rs);
   else w4_rows_kernel<4, 1, 8, GROUP != 32, GROUP, EPI, OUT><<<(nb + 3) / 4, 512, 0, stream>>>(a, sc, rs);
 }

@@ -92,6 +92,31 @@ def test_every_form(monkeypatch, group, mb, nt):
 
 
 @gpu
+@pytest.mark.parametrize("n,k,group", [(4096, 160, 32), (12288, 96, 32), (12304, 160, 32), (4096, 192, 64), (4112, 320, 64), (16400, 128, 64), (4096, 256, 128), (4112, 512, 128),
+                                       (5120, 384, 128), (16384, 256, 128)])
+def test_up_to_16_rows_on_both_sides_of_a_border(n, k, group):
+    """A workgroup has one, two or four blocks of 16 rows of w by their number alone: stored, gated, and into the residual stream."""
+    w, g = pack_w4(*_matrix(n, n, k, group)), torch.Generator().manual_seed(n)
+    found = []
+    for m in (1, 16):
+        x = _x(7, 16, k)[:m]
+        want, tol = _in_64(x, w, out_half=0.0)
+        for out, half in ((torch.bfloat16, 2.0**-8), (torch.float32, 2.0**-24)):
+            got = gemm_w4(x.to(DEV), _to(w, DEV), out)
+            assert ((got.cpu().double() - want).abs() <= tol + half * (want.abs() + tol)).all()
+        found.append(got)
+        gated, gated_tol = _in_64(x, w, gated=True)
+        assert ((gemm_w4(x.to(DEV), _to(w, DEV), silu_mul_epilogue=True).cpu().double() - gated).abs() <= gated_tol).all()
+        h, norm = torch.randn(m, n, generator=g), 1 + 0.1 * torch.randn(n, generator=g)
+        stream = h.to(DEV)
+        rows = weight4.gemm_w4_residual(x.to(DEV), _to(w, DEV), stream, norm.to(DEV), 1e-5).rows
+        want, tol = h.double() + want, tol + 2.0**-24 * (h.double() + want).abs()
+        assert ((stream.cpu().double() - want).abs() <= tol).all()
+        assert ((rows.cpu().double() - want * norm.double()).abs() <= norm.double().abs() * (tol * 1.01 + want.abs() * 1.01 * 2.0**-8)).all()
+    assert torch.equal(found[0], found[1][:1])  # whatever is beside it
+
+
+@gpu
 @pytest.mark.parametrize("group", [64, 128])
 def test_two_blocks_a_wave_have_the_bits_of_one(monkeypatch, group):
     n, k = 1008, 1280
