@@ -137,3 +137,52 @@ def test_wide_matrices_as_they_are_planned(n, k, group, m):
     x = _x(m, m, k)
     want, tol = _in_64(x, w, gated=True)
     assert ((gemm_w4(x.to(DEV), _to(w, DEV), silu_mul_epilogue=True).cpu().double() - want).abs() <= tol).all()
+
+
+@gpu
+def test_cut_products_in_two_graphs_and_on_another_stream():
+    """Sums of a cut K, x in fp16 and its exponents are a call's own: two graphs replayed in turns with eager work between them, and calls on two streams at once."""
+    n, k = 528, 4096
+    w = _to(pack_w4(*_matrix(3, n, k, 128)), DEV)
+    calls = {"wide": (48, lambda x: gemm_w4(x, w)), "large": (200, lambda x: gemm_w4(x, w)), "gated": (40, lambda x: gemm_w4(x, w, silu_mul_epilogue=True)),
+             "sums": (64, lambda x: gemm_w4(x, w, leave_sums=True)), "one row": (1, lambda x: gemm_w4(x, w, torch.float32))}
+    assert weight4.w4_plan(48, n, k, 128)[2] > 1 and weight4.w4_large_plan(200, n, k)[1] > 1
+    xs = {name: [_x(i, m, k).to(DEV) for i in range(3)] for name, (m, _) in calls.items()}
+    want = {name: [call(x).clone() for x in xs[name]] for name, (_, call) in calls.items()}
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for name, (_, call) in calls.items():
+        with torch.cuda.stream(side):
+            there = call(xs[name][1])
+        here = call(xs[name][2])
+        torch.cuda.current_stream().wait_stream(side)
+        assert torch.equal(there, want[name][1]) and torch.equal(here, want[name][2]), name
+    torch.cuda.synchronize()
+    graphs = []
+    for name, (_, call) in calls.items():
+        static, graph = xs[name][0].clone(), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = call(static)
+        graphs.append((name, static, graph, y))
+    for i in (1, 2, 0, 1):
+        for name, static, graph, y in graphs:
+            static.copy_(xs[name][i])
+            y.zero_()
+        for name, static, graph, y in graphs:
+            graph.replay()
+            gemm_w4(xs["wide"][0], w)  # eager work in between
+        torch.cuda.synchronize()
+        for name, static, graph, y in graphs:
+            assert torch.equal(y, want[name][i]), (name, i)
+
+
+@gpu
+@pytest.mark.parametrize("m", [1, 33, 130])
+def test_the_first_rows_are_a_matrix(m):
+    """A view of a packed matrix multiplies as one that was packed from these rows."""
+    n, first, k = 208, 96, 256
+    codes, scales, zeros = _matrix(5, n, k, 64)
+    part, x = _to(pack_w4(codes, scales, zeros), DEV).first_rows(first), _x(m, m, k).to(DEV)
+    whole = _to(pack_w4(codes[:first], scales[:first], zeros[:first]), DEV)
+    assert part.data.data_ptr() and torch.equal(gemm_w4(x, part), gemm_w4(x, whole))
+    assert torch.equal(gemm_w4(x, part, torch.float32), gemm_w4(x, whole, torch.float32))
