@@ -19,7 +19,7 @@ import torch
 from ..kernels.ops import gemm_f32_scratch, gemm_large_scratch, key_parts_scratch
 from ..sampling import Sampler, SamplingParams
 from .context import StepEntry
-from .model import Model
+from .model import Model, matrices4
 from .runner import ModelRunner
 from .scheduler import PENDING, PlannedEntry, Request, Scheduler
 
@@ -61,7 +61,7 @@ def step_memory_estimate(model: Model, max_step_tokens: int, max_batch: int) -> 
                     scratch = max(scratch, gemm_f32_scratch(max_step_tokens, *shape) + cut)
                 elif getattr(v, "packed", None) is not None:
                     scratch = max(scratch, gemm_large_scratch(max_step_tokens, shape[0]))
-    scratch = max([scratch] + [m.scratch_bytes(max_step_tokens) for m in model.matrices4()])
+    scratch = max([scratch] + [m.scratch_bytes(max_step_tokens) for m in matrices4(model.parts.all_parts[1:-1])])
     return int(max_step_tokens * 12 * widest + 3 * max_batch * model.vocab_size * 4) + scratch
 
 

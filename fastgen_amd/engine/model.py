@@ -44,6 +44,13 @@ class ModelParts:
         return dict(self.head.duplicates()) if hasattr(self.head, "duplicates") else {}
 
 
+def matrices4(parts: Sequence[Any]) -> List[Matrix4]:
+    """The matrices in 4 bits of these parts, and of their own parts (a mixture's shared expert), each once."""
+    inner = [v for p in parts for v in vars(p).values() if isinstance(v, Part)]
+    found = (v for p in [*parts, *inner] for v in vars(p).values() if isinstance(v, Matrix4))
+    return list({id(v): v for v in found}.values())
+
+
 def build_parts(layout: ModelLayout) -> ModelParts:
     """Every part of the layout, looked up by kind; nothing is on a device yet."""
     embed = build_part("embedding", layout.embed)
@@ -165,10 +172,7 @@ class Model:
         return all(getattr(p, "capturable", True) for p in self.parts.all_parts)
 
     def matrices4(self) -> List[Matrix4]:
-        """The matrices in 4 bits, those of a part's own parts (a mixture's shared expert) among them, each once."""
-        inner = [v for p in self.parts.all_parts for v in vars(p).values() if isinstance(v, Part)]
-        found = (v for p in self.parts.all_parts + inner for v in vars(p).values() if isinstance(v, Matrix4))
-        return list({id(v): v for v in found}.values())
+        return matrices4(self.parts.all_parts)
 
     def packed(self) -> bool:
         """Whether the matrices have their second copy in the streaming kernels' order."""
